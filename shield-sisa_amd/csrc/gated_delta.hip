@@ -14,10 +14,10 @@
 // of S, V, U and O do not mix, so a wave owns 16 of them and carries its part of S in registers.
 //
 // Every product runs on v_mfma_f32_16x16x32_bf16 with operands split into bf16 parts, fp32 sums: inputs exactly (bf16
-// one part, fp16 two, fp32 three), what is computed on the way -- S, U, T, A -- as three parts, fp32's own precision,
-// since it reaches the state and the gates' gradients, which are fp32 in every mode.  Where a product reaches only o
-// in fp16 or bf16, two parts (2^-17 of a value) are far below o's own rounding.  bf16 parts have fp32's range, so
-// nothing is scaled.
+// one part, fp16 two, fp32 three), what is computed on the way -- S, U, T, A -- as three parts, fp32's own precision.
+// That holds for what reaches only an fp16 or bf16 o as well: where a token replaces what its key held, Q S and A U
+// cancel, and what two parts leave out (2^-17 of them) is then no longer below o's own rounding.  bf16 parts have fp32's
+// range, so nothing is scaled.
 //
 // Fragment orders.  The contraction index of a product may be visited in any order as long as both operands agree.  A
 // result fragment holds, per lane (g, r), column r and rows 4 g .. 4 g + 3 of a 16-row tile; an operand fragment wants
@@ -35,10 +35,10 @@ namespace {
 typedef float f32x8v __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-template <typename T> struct Parts;            // bf16 parts of an input; of what reaches only o; tokens per chunk
-template <> struct Parts<bf16> { static constexpr int IN = 1, OUT = 2, C = 64; };
-template <> struct Parts<f16> { static constexpr int IN = 2, OUT = 2, C = 64; };
-template <> struct Parts<float> { static constexpr int IN = 3, OUT = 3, C = 32; };
+template <typename T> struct Parts;            // bf16 parts of an input; tokens per chunk
+template <> struct Parts<bf16> { static constexpr int IN = 1, C = 64; };
+template <> struct Parts<f16> { static constexpr int IN = 2, C = 64; };
+template <> struct Parts<float> { static constexpr int IN = 3, C = 32; };
 constexpr int MID = 3;                         // bf16 parts of everything else
 
 constexpr int kBlock = 1024;   // bytes of a 16 x 32 fragment block
@@ -56,7 +56,7 @@ __device__ __forceinline__ constexpr int tri_up(int i, int s) { return s * (s + 
 template <typename T> struct Record {   // what delta_chunk_kernel leaves per (chunk, head): T^T, vectors, A^T
     static constexpr int C = Parts<T>::C, NT = C / 16, NP = C / 32, BLOCKS = NP * (NP + 1), MAT = BLOCKS * kBlock;
     static constexpr int VEC_AT = MID * MAT, A_AT = VEC_AT + kBlock;   // vectors: exp G, exp(G_C - G), b, C floats each; exp G_C
-    static constexpr int bytes(int a_parts) { return A_AT + a_parts * MAT; }
+    static constexpr int BYTES = A_AT + MID * MAT;
     static_assert(3 * C * 4 + 16 <= kBlock, "the vectors' block");
 };
 
@@ -332,7 +332,7 @@ template <> struct Plain<float> {
 // column; the blocks below them column by column, T_ij = -T_ii sum_k L_ik T_kj, in fp32 on the matrix cores.
 // Memory and the chain of substitutions share the time: 257 chunks x 8 heads of 128 keys in bf16 take 31 us, 38 MB read and
 // 65 MB of records written, 3.3 TB/s; many small workgroups hide the chains of each other.
-template <typename T, int NK, int A_PARTS, bool WHOLE>
+template <typename T, int NK, bool WHOLE>
 __global__ void __launch_bounds__(256) delta_chunk_kernel(DeltaOp a) {
     typedef Record<T> R;
     typedef Plain<T> X;
@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(256) delta_chunk_kernel(DeltaOp a) {
     }
     __syncthreads();   // the tiles are read; their memory now holds L's columns
     float(*lt)[PITCH] = reinterpret_cast<float(*)[PITCH]>(mem);
-    unsigned char* rec = a.records + (it.slot * a.h + head) * R::bytes(A_PARTS);
+    unsigned char* rec = a.records + (it.slot * a.h + head) * R::BYTES;
     const int col = row_of(j, r);
     const double gc = gsum[col];
 #pragma unroll
@@ -436,10 +436,10 @@ __global__ void __launch_bounds__(256) delta_chunk_kernel(DeltaOp a) {
             if (first == 0) *reinterpret_cast<f32x4*>(&lt[col][row]) = l[n];
         }
         if (first + BOTH == 2) {
-            bf16x8 part[A_PARTS];
-            split8<A_PARTS>(q[0], q[1], part);
+            bf16x8 part[MID];
+            split8<MID>(q[0], q[1], part);
 #pragma unroll
-            for (int p = 0; p < A_PARTS; ++p)
+            for (int p = 0; p < MID; ++p)
                 *reinterpret_cast<bf16x8*>(rec + R::A_AT + p * R::MAT + tri_up(j, s) * kBlock + at) = part[p];
         }
     }
@@ -516,16 +516,19 @@ __global__ void __launch_bounds__(256) delta_chunk_kernel(DeltaOp a) {
 // of v or d_o, the record.  Where the inputs are already what the tiles hold (bf16, WHOLE) everything goes straight to
 // LDS; else K and Q wait in registers and are converted and stored when the step ends -- into the other stage, or, where
 // two do not fit, into their own place behind one more barrier.  X of two bytes goes through LDS as well (the
-// transposing read hands a lane four tokens of its column), X of four bytes and unaligned X through registers.
+// transposing read hands a lane four tokens of its column), X of four bytes and unaligned X through registers.  Where two
+// stages of X do not fit either, it has one, and a barrier between the step's own read of it and the fetch (xs_read).
 template <typename T, int NK, int W, bool WHOLE, bool WITH_Q, int REC> struct Feed {
     typedef Record<T> R;
     typedef RowTile<T, NK, 64 * W> Tile;
     static constexpr int C = R::C, NT = R::NT;
     static constexpr bool DIRECT = WHOLE && sizeof(T) == 2 && Parts<T>::IN == 1, X_LDS = WHOLE && sizeof(T) == 2;
     static constexpr int KQ = (WITH_Q ? 2 : 1) * Tile::BYTES, X_BYTES = X_LDS ? NT * (W / 2) * kBlock : 0;
-    static constexpr bool TWO = 2 * (KQ + X_BYTES + REC) <= 160 * 1024;
-    static constexpr int STAGE = X_BYTES + REC, BYTES = (TWO ? 2 : 1) * KQ + 2 * STAGE;
-    static_assert(BYTES <= 160 * 1024 && (TWO || !DIRECT), "LDS");
+    static constexpr bool TWO = DIRECT || 2 * (KQ + X_BYTES + REC) <= 160 * 1024;
+    static constexpr int TILES = (TWO ? 2 : 1) * KQ;
+    static constexpr bool TWO_X = TILES + 2 * (X_BYTES + REC) <= 160 * 1024;
+    static constexpr int BYTES = TILES + 2 * REC + (TWO_X ? 2 : 1) * X_BYTES;
+    static_assert(BYTES <= 160 * 1024, "LDS");
     unsigned char* mem;
     const T *k, *q, *x;         // the head's rows at the sequence's first token
     const unsigned char* rec;   // the head's record of the sequence's first chunk
@@ -537,8 +540,8 @@ template <typename T, int NK, int W, bool WHOLE, bool WITH_Q, int REC> struct Fe
 
     __device__ __forceinline__ unsigned char* k_tile(int st) const { return mem + (TWO ? st * KQ : 0); }
     __device__ __forceinline__ unsigned char* q_tile(int st) const { return k_tile(st) + Tile::BYTES; }
-    __device__ __forceinline__ unsigned char* x_tile(int st) const { return mem + (TWO ? 2 : 1) * KQ + st * STAGE; }
-    __device__ __forceinline__ unsigned char* record(int st) const { return x_tile(st) + X_BYTES; }
+    __device__ __forceinline__ unsigned char* record(int st) const { return mem + TILES + st * REC; }
+    __device__ __forceinline__ unsigned char* x_tile(int st) const { return mem + TILES + 2 * REC + (TWO_X ? st * X_BYTES : 0); }
 
     __device__ __forceinline__ void rows(const T* base, long long stride, int valid, unsigned char* tile) const {
         const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
@@ -615,6 +618,10 @@ template <typename T, int NK, int W, bool WHOLE, bool WITH_Q, int REC> struct Fe
                 for (int e = 0; e < 4; ++e) v[i][e] = float(xr[i][e]);
             }
         }
+    }
+    // Every wave has its columns of X and the next step's may take their place.  LDS alone: the loads ahead stay in flight.
+    __device__ __forceinline__ void xs_read() const {
+        if constexpr (!TWO_X) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     }
     // X in registers moves on: what was fetched becomes the current step's, so that the next fetch can be issued
     __device__ __forceinline__ void advance() {
@@ -756,7 +763,7 @@ __global__ void __launch_bounds__(64 * W) delta_transit_kernel(DeltaOp a) {
     if (!item_of(a, slots_of(a, seg_tokens(a, C)), a.h, slices, &it)) return;
     const int slice = it.slice, head = it.head;
     const long long slot = it.slot;
-    constexpr long long REC = R::bytes(TRAIN ? MID : Parts<T>::OUT);
+    constexpr long long REC = R::BYTES;
     const bool find_m = slice * W + wave >= vtiles, with_v = slice * W < vtiles;   // this wave; any of the workgroup
     Piece p;   // the returns are uniform over the workgroup
     if (!piece_of(a, slot, seg_tokens(a, C), &p) || p.len <= seg_tokens(a, C)) return;
@@ -952,9 +959,9 @@ __global__ void __launch_bounds__(64 * NK) delta_join_kernel(DeltaOp a, const fl
 template <typename T, int NK, int W, bool TRAIN, bool WHOLE>
 __global__ void __launch_bounds__(64 * W) delta_scan_kernel(DeltaOp a) {
     typedef Record<T> R;
-    constexpr int C = R::C, NT = R::NT, NP = R::NP, P = Parts<T>::IN, OUT = Parts<T>::OUT, M = 2 * NK;
-    typedef Feed<T, NK, W, WHOLE, true, R::bytes(OUT)> Reader;
-    constexpr long long REC = R::bytes(TRAIN ? MID : OUT);
+    constexpr int C = R::C, NT = R::NT, NP = R::NP, P = Parts<T>::IN, M = 2 * NK;
+    typedef Feed<T, NK, W, WHOLE, true, R::BYTES> Reader;
+    constexpr long long REC = R::BYTES;
     __shared__ __attribute__((aligned(1024))) unsigned char mem[Reader::BYTES];
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1060,16 +1067,13 @@ __global__ void __launch_bounds__(64 * W) delta_scan_kernel(DeltaOp a) {
         for (int s = 0; s < NP; ++s) split8<MID>(x[2 * s], x[2 * s + 1], rf[s]);
 #pragma unroll
         for (int s = 0; s < NK; ++s) {
-            bf16x8 so[OUT];
-#pragma unroll
-            for (int n = 0; n < OUT; ++n) so[n] = sf[s][n];
             if (s + 1 < NK) read_rows<P, NT, NK>(qt + at, s + 1, qf[(s + 1) & 1]);
-            mul_t(so, qf[s & 1], o);
+            mul_t(sf[s], qf[s & 1], o);
         }
         fence();
         in.fetch_piece(1, next, st ^ 1, true);   // Q
         read_lower<MID, NT, R::MAT>(rec + at_t, 0, tf);
-        bf16x8 af[NT][OUT];
+        bf16x8 af[NT][MID];
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
             x[i] = f32x4{0, 0, 0, 0};
@@ -1081,9 +1085,10 @@ __global__ void __launch_bounds__(64 * W) delta_scan_kernel(DeltaOp a) {
             mul_tri<true>(s, tf, rf[s], x);
         }
         fence();
+        in.xs_read();
         in.fetch_piece(2, next, st ^ 1, true);   // X
         in.fetch_piece(3, next, st ^ 1, true);   // the record
-        read_lower<OUT, NT, R::MAT>(rec + R::A_AT + at_t, 0, af);
+        read_lower<MID, NT, R::MAT>(rec + R::A_AT + at_t, 0, af);
         fence();
 #pragma unroll
         for (int s = 0; s < NP; ++s) split8<MID>(x[2 * s], x[2 * s + 1], rf[s]);   // U
@@ -1100,13 +1105,10 @@ __global__ void __launch_bounds__(64 * W) delta_scan_kernel(DeltaOp a) {
         for (int m = 0; m < M; ++m) S[m] *= all;
 #pragma unroll
         for (int s = 0; s < NP; ++s) {
-            bf16x8 uo[OUT];
-#pragma unroll
-            for (int n = 0; n < OUT; ++n) uo[n] = rf[s][n];
-            if (s) read_lower<OUT, NT, R::MAT>(rec + R::A_AT + at_t, s, af);
-            mul_tri_t(s, uo, af, o);
+            if (s) read_lower<MID, NT, R::MAT>(rec + R::A_AT + at_t, s, af);
+            mul_tri_t(s, rf[s], af, o);
         }
-        interleave<R::BLOCKS * (OUT == 2 ? 3 : 6), 6>();
+        interleave<R::BLOCKS * 6, 6>();
         fence();
         add_outer<P, M, NK, NT>(kt + at_t, lf, S);
 #pragma unroll
@@ -1243,7 +1245,7 @@ template <typename T, int NK, int W, bool FIND, bool WHOLE>
 __global__ void __launch_bounds__(64 * W) delta_back_kernel(DeltaOp a, DeltaGrad d) {
     typedef Record<T> R;
     constexpr int C = R::C, NT = R::NT, NP = R::NP, P = Parts<T>::IN, M = 2 * NK;
-    typedef Feed<T, NK, W, WHOLE, true, R::bytes(MID)> Reader;
+    typedef Feed<T, NK, W, WHOLE, true, R::BYTES> Reader;
     __shared__ __attribute__((aligned(1024))) unsigned char mem[Reader::BYTES];
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1264,8 +1266,8 @@ __global__ void __launch_bounds__(64 * W) delta_back_kernel(DeltaOp a, DeltaGrad
     in.k = static_cast<const T*>(a.k) + p.begin * a.k_stride + hq * a.k_head;
     in.q = static_cast<const T*>(a.q) + p.begin * a.q_stride + hq * a.q_head;
     in.x = static_cast<const T*>(d.d_o) + (p.begin * a.h + head) * a.dv;
-    in.rec_stride = a.h * (long long)R::bytes(MID);
-    in.rec = a.records + slot0 * in.rec_stride + head * (long long)R::bytes(MID);
+    in.rec_stride = a.h * (long long)R::BYTES;
+    in.rec = a.records + slot0 * in.rec_stride + head * (long long)R::BYTES;
     in.k_stride = a.k_stride;
     in.q_stride = a.q_stride;
     in.x_stride = (long long)a.h * a.dv;
@@ -1431,7 +1433,7 @@ __global__ void __launch_bounds__(512) delta_grad_kernel(DeltaOp a, DeltaGrad d)
     };
     float rv = 0.0f, gv = 0.0f;   // the next head's vectors and g
     const auto fetch_head = [&](int head) {
-        const float* rec = reinterpret_cast<const float*>(a.records + (it.slot * a.h + head) * R::bytes(MID) + R::VEC_AT);
+        const float* rec = reinterpret_cast<const float*>(a.records + (it.slot * a.h + head) * R::BYTES + R::VEC_AT);
         if (wave == 0 && lane < valid) gv = a.g[(begin + lane) * a.g_stride + head];
         if (tid < 3 * C + 1) rv = rec[tid];
     };
@@ -1806,7 +1808,7 @@ DeltaSizes delta_sizes(OpType t, const DeltaOp& a, bool train) {
         typedef decltype(type) T;
         const size_t slots = size_t(slots_on_host(a, Parts<T>::C)) * size_t(a.h), block = size_t(MID) * kBlock;
         const size_t vtiles = 2 * ((size_t(a.dv) + 31) / 32), nk = a.dk <= 64 ? 2 : 4;
-        s.records = slots * Record<T>::bytes(train ? MID : Parts<T>::OUT);
+        s.records = slots * Record<T>::BYTES;
         if (train) {
             s.starts = slots * vtiles * 2 * nk * kBlock;
             s.u = slots * vtiles * Record<T>::NT * kBlock;
@@ -1850,7 +1852,7 @@ void launch_delta_fwd(OpType t, DeltaOp a, bool train, hipStream_t s) {
                 for_flag(whole_rows(t, a), [&](auto whole) {
                     constexpr bool TRAIN = training.value, WHOLE = whole.value;
                     constexpr int NK = nk.value, C = Parts<T>::C;
-                    delta_chunk_kernel<T, NK, TRAIN ? MID : Parts<T>::OUT, WHOLE>
+                    delta_chunk_kernel<T, NK, WHOLE>
                         <<<dim3(item_grid(slots_on_host(a, C), a.h, 1)), dim3(256), 0, s>>>(a);
                     if (a.segment * C < a.n_tokens) {
                         for_flag(wide && WHOLE, [&](auto both) {

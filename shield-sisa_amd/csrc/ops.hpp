@@ -74,7 +74,7 @@ struct DeltaOp {
     unsigned char *records, *starts, *u;
     // sequences cut into segments of this many chunks: the segments' transitions M and N and the states between them
     long long segment;
-    unsigned char *seg_m, *seg_mt, *seg_n, *seg_s;   // (seg_mt: M^T, for training)
+    unsigned char *seg_m, *seg_mt, *seg_n, *seg_s;   // (seg_mt: M^T, for training; a backward call has seg_n, seg_s of its own)
 };
 
 struct DeltaGrad {

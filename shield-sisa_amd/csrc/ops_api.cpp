@@ -174,6 +174,8 @@ void delta_inputs(const shv::DeltaOp& d) {
 size_t scan_bytes(const shv::DeltaSizes& s, bool train) {
     return s.records + s.starts + s.u + (train ? 2 : 1) * s.seg_m + 2 * s.seg_n;
 }
+// ... and the backward pass's: `saved` is only read there, so it has its own seg_n and seg_s.
+size_t back_bytes(const shv::DeltaSizes& s) { return s.starts + s.u + 2 * s.seg_n; }
 void scan_memory(const shv::DeltaSizes& s, void* p, shv::DeltaOp* d) {
     d->records = static_cast<unsigned char*>(p);
     d->starts = d->records + s.records;
@@ -194,7 +196,7 @@ int shv_hip_gated_delta_sizes(const shv_hip_delta_args* a, int train, size_t* wo
         shv::DeltaOp d;
         const shv::OpType t = delta_args(a, &d);
         const shv::DeltaSizes s = shv::delta_sizes(t, d, train != 0);
-        *workspace = train ? s.starts + s.u : shv::delta_by_token(d) ? 0 : scan_bytes(s, false);
+        *workspace = train ? back_bytes(s) : shv::delta_by_token(d) ? 0 : scan_bytes(s, false);
         *saved = train ? scan_bytes(s, true) : 0;
     });
 }
@@ -237,7 +239,7 @@ int shv_hip_gated_delta_backward(const shv_hip_delta_args* a, const shv_hip_delt
         require(a->saved != nullptr && a->saved_bytes >= scan_bytes(s, true), "saved too small");
         aligned_to(a->saved, 256, "saved");
         scan_memory(s, a->saved, &d);
-        require(a->workspace && a->workspace_bytes >= s.starts + s.u, "workspace too small");
+        require(a->workspace && a->workspace_bytes >= back_bytes(s), "workspace too small");
         aligned_to(a->workspace, 256, "workspace");
         aligned_to(g->d_o, ts, "d_o");
         aligned_to(g->d_q, ts, "d_q");
@@ -258,6 +260,8 @@ int shv_hip_gated_delta_backward(const shv_hip_delta_args* a, const shv_hip_delt
         b.d_state_in = g->d_state_in;
         b.ends = static_cast<unsigned char*>(a->workspace);
         b.dr = b.ends + s.starts;
+        d.seg_n = b.dr + s.u;
+        d.seg_s = d.seg_n + s.seg_n;
         launch([&] { shv::launch_delta_bwd(t, d, b, static_cast<hipStream_t>(stream)); });
     });
 }

@@ -51,8 +51,8 @@ struct NormBwd {
 
 constexpr int kNormMaxN = 8192;
 int norm_bwd_groups(long long rows, int n);
-void launch_norm_fwd(OpType t, const NormFwd& a, hipStream_t s);
-void launch_norm_bwd(OpType t, const NormBwd& a, hipStream_t s);
+void launch_norm_fwd(OpType t, NormFwd a, hipStream_t s);
+void launch_norm_bwd(OpType t, NormBwd a, hipStream_t s);
 
 // ---- the gated delta rule (gated_delta.hip)
 constexpr int kDeltaMaxK = 128, kDeltaMaxV = 256;

@@ -188,7 +188,7 @@ struct Item {
 constexpr int kXcds = 8;
 __device__ __forceinline__ bool item_of(const DeltaOp& a, long long slots, int heads, int slices, Item* it) {
     const int group = heads / a.hk;
-    const unsigned n = unsigned(slots * heads * slices), per = (n + kXcds - 1) / kXcds;   // the host keeps it below 2^31
+    const unsigned n = unsigned(slots * heads * slices), per = (n + kXcds - 1) / kXcds;   // (delta_launches keeps it small)
     unsigned id = blockIdx.x % kXcds * per + blockIdx.x / kXcds;
     if (blockIdx.x / kXcds >= per || id >= n) return false;
     it->slice = int(id % unsigned(slices));
@@ -1829,6 +1829,20 @@ DeltaSizes delta_sizes(OpType t, const DeltaOp& a, bool train) {
 bool delta_by_token(const DeltaOp& a) {
     const long long most = (long long)a.n_seqs * a.h >= 256 ? 32 : 12, longest = a.offsets ? a.max_len : a.per_seq;
     return longest <= most && (!a.offsets || a.max_len > 0);
+}
+
+// Whether every launch of a call has fewer than 2^32 threads, HIP's limit; items and workgroups then fit 32 bits by far.
+bool delta_launches(OpType t, DeltaOp a, bool train) {
+    const auto fits = [](long long groups, int threads) { return (groups + kXcds) * threads < (1LL << 32); };
+    if (!train && delta_by_token(a)) return fits(((long long)a.n_seqs * a.h * ((a.dv + 31) / 32) + 3) / 4, 256);
+    a.segment = segment_of(t, a, train);
+    const long long C = t == OpType::F32 ? 32 : 64, slots = slots_on_host(a, C), segs = slots_on_host(a, C * a.segment);
+    const int vtiles = 2 * ((a.dv + 31) / 32), keys = a.dk <= 64 ? 4 : 8, nk = keys / 2;
+    const auto sliced = [&](int tiles, int waves) { return fits(segs * a.h * ((tiles + waves - 1) / waves), 64 * waves); };
+    bool ok = fits(slots * a.h, 256) && sliced(vtiles, 4) && sliced(vtiles, 8);
+    if (a.segment * C < a.n_tokens)
+        ok = ok && sliced(vtiles + keys, keys) && sliced(vtiles + keys, 2 * keys) && fits((long long)a.n_seqs * a.h * vtiles, 64 * nk);
+    return ok && (!train || fits(slots * a.hk, 512));
 }
 
 void launch_delta_fwd(OpType t, DeltaOp a, bool train, hipStream_t s) {

@@ -92,6 +92,7 @@ struct DeltaSizes {   // bytes; starts and u are also those of the backward pass
 };
 DeltaSizes delta_sizes(OpType t, const DeltaOp& a, bool train);
 bool delta_by_token(const DeltaOp& a);   // the recurrent kernel serves this call: no work memory
+bool delta_launches(OpType t, DeltaOp a, bool train);   // the call's launches are no larger than HIP takes
 void launch_delta_fwd(OpType t, DeltaOp a, bool train, hipStream_t s);
 void launch_delta_bwd(OpType t, DeltaOp a, const DeltaGrad& d, hipStream_t s);
 

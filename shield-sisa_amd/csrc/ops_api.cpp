@@ -102,6 +102,7 @@ size_t norm_work_bytes(const shv::NormFwd& f) {
 }
 
 // ------------------------------------------------------------------------------------------ the gated delta rule
+constexpr const char* kTooMany = "too many sequences, heads or tokens for one call";
 shv::OpType delta_args(const shv_hip_delta_args* a, shv::DeltaOp* d) {
     require(a != nullptr, "null argument");
     const shv::OpType t = type_of(a->mode);
@@ -115,7 +116,7 @@ shv::OpType delta_args(const shv_hip_delta_args* a, shv::DeltaOp* d) {
     require(a->max_len >= 0, "max_len out of range");
     require(a->d_offsets || a->n_tokens % a->n_seqs == 0, "without offsets, n_tokens has to be a multiple of n_seqs");
     require((long long)a->n_seqs * a->heads * 16 < (1LL << 31) && a->n_tokens / 32 + a->n_seqs < (1LL << 31),
-            "too many sequences, heads or tokens for one call");
+            kTooMany);
     require(std::isfinite(a->scale), "scale has to be finite");
     require(a->n_states >= 0, "state count out of range");
     aligned_to(a->d_offsets, 8, "d_offsets");
@@ -195,6 +196,7 @@ int shv_hip_gated_delta_sizes(const shv_hip_delta_args* a, int train, size_t* wo
         require(workspace && saved, "null argument");
         shv::DeltaOp d;
         const shv::OpType t = delta_args(a, &d);
+        require(shv::delta_launches(t, d, train != 0), kTooMany);
         const shv::DeltaSizes s = shv::delta_sizes(t, d, train != 0);
         *workspace = train ? back_bytes(s) : shv::delta_by_token(d) ? 0 : scan_bytes(s, false);
         *saved = train ? scan_bytes(s, true) : 0;
@@ -208,6 +210,7 @@ int shv_hip_gated_delta(const shv_hip_delta_args* a, void* stream) {
         delta_inputs(d);
         require(d.n_tokens == 0 || d.o, "null argument: o");
         const bool train = a->saved != nullptr;
+        require(shv::delta_launches(t, d, train), kTooMany);
         if (train) {
             require(!d.state_in || d.state_in != d.state_out, "a call that trains cannot store over state_in");
             const shv::DeltaSizes s = shv::delta_sizes(t, d, true);
@@ -235,6 +238,7 @@ int shv_hip_gated_delta_backward(const shv_hip_delta_args* a, const shv_hip_delt
                 "null argument: d_o, d_q, d_k, d_v, d_g or d_beta");
         // a sequence's first and last segments are worked on at the same time
         require(!g->d_state_in || g->d_state_in != g->d_state_out, "d_state_in cannot be d_state_out");
+        require(shv::delta_launches(t, d, true), kTooMany);
         const shv::DeltaSizes s = shv::delta_sizes(t, d, true);
         require(a->saved != nullptr && a->saved_bytes >= scan_bytes(s, true), "saved too small");
         aligned_to(a->saved, 256, "saved");

@@ -45,3 +45,37 @@ def test_outputs_whose_terms_cancel(shv, mode, n, dk, dv):
             assert float(want["o"][::2].abs().max()) > 0.3 * top and float(w.abs().max()) < 1e-3 * top
             bad = (o - w).abs() - (1e-6 * top + base.ULP[mode] * w.abs())
             assert float(bad.max()) <= 0, (state, max_len, float((o - w).abs().max() / top))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mode", base.MODES)
+@pytest.mark.parametrize("lens,h,dk,dv", [([70, 9], 2, 64, 64), ([130], 2, 128, 128), ([70, 9], 2, 40, 24), ([1900], 2, 64, 96)],
+                         ids=str)
+def test_fp32_outputs_have_fp32_precision(shv, mode, lens, h, dk, dv):
+    """States, their gradients and those of g and beta are fp32 in every mode, and the inputs are exact: they are held to
+    what fp32 inputs are held to (test_gated_delta.py: 1e-5, gradients 3 times that, g's 10 times)."""
+    s = base.make(mode, lens, h, h, dk, dv, seed=53, decay=0.01)
+    want, grads = base.reference(s, True, True)
+    got = base.forward(shv, s, "states")["state"].cpu()
+    base.close(got, want["state"], 1e-5, 0.0, "state")
+    out, got = base.backward(shv, s)
+    base.close(out["state"].cpu(), want["state"], 1e-5, 0.0, "state of a training call")
+    base.close(got["state"].cpu(), grads["state"], 3e-5, 0.0, "gradient of the state")
+    for n, tol in (("beta", 3e-5), ("g", 1e-4)):
+        for i, (a, b) in enumerate(zip(base.by_seq(s, got[n].cpu()), base.by_seq(s, grads[n]))):
+            base.close(a, b, tol, 0.0, f"gradient of {n}, sequence {i}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mode", ["fp32", "bf16"])   # (o passes fp16's range here)
+@pytest.mark.parametrize("lens,most,dk", [([64, 3], 1.0, 64), ([150], 0.5, 40), ([1100], 0.06, 64)], ids=str)
+def test_growing_states(shv, mode, lens, most, dk):
+    """g above 0: right while exp of its sum over any run of tokens is finite (here up to exp(64))."""
+    s = base.make(mode, lens, 1, 2, dk, 48, seed=54)
+    s["g"] = most * torch.rand(s["g"].shape, generator=torch.Generator().manual_seed(55))
+    if lens[0] == 64:
+        s["g"][:64] = most
+    assert float(s["g"].double().sum(0).max()) < 80
+    want, _ = base.reference(s)
+    for max_len in (0, 1):
+        base.check(s, base.forward(shv, s, f"growing, max_len {max_len}", max_len=max_len), want, mode)

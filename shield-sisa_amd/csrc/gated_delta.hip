@@ -603,16 +603,27 @@ template <typename T, int NK, int W, bool WHOLE, bool WITH_Q, int REC> struct Fe
 #pragma unroll
         for (int piece = 0; piece < 4; ++piece) fetch_piece(piece, c, st, with_x);
     }
-    // the X columns of the step that fetch prepared
-    __device__ __forceinline__ void columns(int st, f32x4* v) {
+    // the X columns of the step that fetch prepared: from LDS as stored, and widened
+    __device__ __forceinline__ void read_x(int st, s16x4* raw) const {
         const int lane = tid & 63, r = lane & 15, g = lane >> 4, wave = tid >> 6;
+        if constexpr (X_LDS) {
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+                raw[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (LdsQuad)((Lds)x_tile(st) + (i * (W / 2) + (wave >> 1)) * kBlock + 16 * slot_of(4 * g + (r >> 2), r & 3) + 8 * (wave & 1)));
+        }
+    }
+    __device__ __forceinline__ void columns(int st, f32x4* v) const {
+        s16x4 raw[NT];
+        read_x(st, raw);
+        widen(raw, v);
+    }
+    __device__ __forceinline__ void widen(const s16x4* raw, f32x4* v) const {
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
             if constexpr (X_LDS) {
                 typedef T T4 __attribute__((ext_vector_type(4)));
-                const s16x4 raw = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (LdsQuad)((Lds)x_tile(st) + (i * (W / 2) + (wave >> 1)) * kBlock + 16 * slot_of(4 * g + (r >> 2), r & 3) + 8 * (wave & 1)));
-                v[i] = __builtin_convertvector(__builtin_bit_cast(T4, raw), f32x4);
+                v[i] = __builtin_convertvector(__builtin_bit_cast(T4, raw[i]), f32x4);
             } else {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[i][e] = float(xr[i][e]);
@@ -1033,9 +1044,12 @@ __global__ void __launch_bounds__(64 * W) delta_scan_kernel(DeltaOp a) {
         for (int i = 0; i < NT; ++i) x[i] = o[i] = f32x4{0, 0, 0, 0};
         // K S, the next block of S split while the products of one run
         bf16x8 sf[NK][MID], kf[2][NT][P];
+        s16x4 xs[NT];
+        if constexpr (!Reader::TWO_X) in.read_x(st, xs);   // here the waves are still together, so the barrier costs least
         read_rows<P, NT, NK>(kt + at, 0, kf[0]);
         split8<MID>(S[0], S[1], sf[0]);
         fence();
+        in.xs_read();
 #pragma unroll
         for (int s = 0; s < NK; ++s) {
             if (s + 1 < NK) {
@@ -1052,7 +1066,8 @@ __global__ void __launch_bounds__(64 * W) delta_scan_kernel(DeltaOp a) {
         // columns of one token and stores them at once
         bf16x8 tf[NT][MID], rf[NP][MID], qf[2][NT][P];
         read_rows<P, NT, NK>(qt + at, 0, qf[0]);
-        in.columns(st, v);
+        if constexpr (Reader::TWO_X) in.read_x(st, xs);
+        in.widen(xs, v);
         f32x4 gam[NT], bet[NT];
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
@@ -1085,7 +1100,6 @@ __global__ void __launch_bounds__(64 * W) delta_scan_kernel(DeltaOp a) {
             mul_tri<true>(s, tf, rf[s], x);
         }
         fence();
-        in.xs_read();
         in.fetch_piece(2, next, st ^ 1, true);   // X
         in.fetch_piece(3, next, st ^ 1, true);   // the record
         read_lower<MID, NT, R::MAT>(rec + R::A_AT + at_t, 0, af);

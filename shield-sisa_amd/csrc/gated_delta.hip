@@ -331,7 +331,7 @@ template <> struct Plain<float> {
 // as they are.  L goes to LDS by columns.  Its 16 x 16 diagonal blocks are inverted by forward substitution, a lane per
 // column; the blocks below them column by column, T_ij = -T_ii sum_k L_ik T_kj, in fp32 on the matrix cores.
 // Memory and the chain of substitutions share the time: 257 chunks x 8 heads of 128 keys in bf16 take 31 us, 38 MB read and
-// 65 MB of records written, 3.3 TB/s; many small workgroups hide the chains of each other.
+// 77 MB of records written, 3.7 TB/s; many small workgroups hide the chains of each other.
 template <typename T, int NK, bool WHOLE>
 __global__ void __launch_bounds__(256) delta_chunk_kernel(DeltaOp a) {
     typedef Record<T> R;
@@ -759,7 +759,8 @@ __device__ __forceinline__ long long seg_tokens(const DeltaOp& a, int C) { retur
 
 // A wave finds 16 columns of N (the first tiles: columns of v) or of M (the others: columns of the identity).  A training
 // call needs M of the last segment as well.  At 128 x 128 the 16 tiles go to two workgroups where each has a compute unit
-// (3.7 us a step), else to one, where they share K and T (5.4 us a step of both; a second round of the halves 7.4).
+// (3.7 us a step), else to one, where they share K and T (5.4 us a step of both; a second round of the halves 7.4).  In fp16
+// the one has 4 registers too few of its 128 and spills them.
 template <typename T, int NK, int W, bool TRAIN, bool WHOLE>
 __global__ void __launch_bounds__(64 * W) delta_transit_kernel(DeltaOp a) {
     typedef Record<T> R;
@@ -963,10 +964,12 @@ __global__ void __launch_bounds__(64 * NK) delta_join_kernel(DeltaOp a, const fl
     }
 }
 
-// W waves, 16 columns of v each, over one segment.  5.2 us a step of 64 tokens at 128 x 128 in bf16 with eight waves: bound by
-// the issue of matrix and vector instructions, which add up (an MFMA 16 cycles, the splits and scalings as much again), and
-// two waves a SIMD more change nothing (fp32 x 64 keys, held to 128 registers: 164 us against 163 for 128 sequences of
-// 321 tokens x 6 heads).  Memory is far off: 150 MB read and 34 MB written in 69 us.
+// W waves, 16 columns of v each, over one segment.  At 128 x 128 in bf16 a step of 64 tokens takes 4.6 us with four waves, and
+// 5 to 6 with eight (232 segments of 9 steps: 77 us).  No unit is busy half of that: the matrix cores 32 %, the vector units
+// 32 %, LDS some 40 % (690 KB a step at 128 bytes a clock: every wave reads K, Q, T and A for its 16 columns); 162 MB read
+// and 34 written are 2.5 TB/s.  A step is a chain -- K S, R, T R, A U, S -- whose links wait for each other inside a wave, and the one or two
+// waves of a SIMD hide too little of it.  Two more, at 128 registers, change nothing (fp32 x 64 keys, 128 sequences of 321
+// tokens x 6 heads: 164 us against 163).  General loads of two-byte types with 128 keys spill 5 registers of 256.
 template <typename T, int NK, int W, bool TRAIN, bool WHOLE>
 __global__ void __launch_bounds__(64 * W) delta_scan_kernel(DeltaOp a) {
     typedef Record<T> R;
@@ -1389,9 +1392,10 @@ __global__ void __launch_bounds__(64 * W) delta_back_kernel(DeltaOp a, DeltaGrad
 // share of the dk tiles, every product transposed so that a lane holds four key dimensions of one token.  U, dR, S and
 // dS' come in as fp32 accumulators, SLAB tiles of v at a time, and are split on the way to LDS: as fp32 they are two
 // thirds of what their parts would be, and this kernel and the scans that feed it move more of them than anything else.
-// 128 chunks x 4 q / k heads x 2 heads x 128 x 128 in bf16 take 125 us: 280 MB read, 50 written, the matrix cores 11 % and
-// the vector units 17 % busy.  Its phases wait for each other at barriers with one workgroup on a compute unit; sixteen
-// waves have too few registers for the accumulators (210 us).
+// 128 chunks x 4 q / k heads x 2 heads x 128 x 128 in bf16 take 126 us: 285 MB read, 50 written, the matrix cores 11 % and
+// the vector units 16 % busy (fp16 x 64 keys, 32 sequences of 321 tokens x 6 heads: 108 us, 14 % and 29 %).  Its phases wait
+// for each other at barriers with one workgroup on a compute unit.  With 128 keys the accumulators leave too few registers
+// even so: 28 of 256 are spilled in the two-byte types, and sixteen waves, of 128, took 210 us.
 template <typename T, int NK, bool WHOLE>
 __global__ void __launch_bounds__(512) delta_grad_kernel(DeltaOp a, DeltaGrad d) {
     typedef Record<T> R;
@@ -1774,12 +1778,16 @@ long long segments_on_host(const DeltaOp& a, long long tokens) {
 // steps: in us at 128 x 128, bf16, a start of 15 and 5.2 a step for the scan, 20 and 5.4 for the transitions (12 and 3.7
 // where their two halves have a compute unit each), 4 and 1.6 a segment for the join; backward both walks together 45 and
 // 7.2 a step, the join 2.6 a segment.  Workgroups that fit into one round of the 256 compute units step together; more of
-// them share the units, each with a start worth 3 steps.  Where lengths differ the counts are bounds and the end is uneven,
+// them share the units, each with a start worth 3 steps.  (The scan's 5.2 were fitted before its o took the third parts; its
+// picks are measured below as they are.)  Where lengths differ the counts are bounds and the end is uneven,
 // so there the gain has to be larger.
-// Measured, split and whole, in us, one sequence of 128 x 128: bf16, 8 heads: 512 tokens 41 and 44, 1,024 49 and 74, 2,048 67
-// and 137, 16,421 224 and 1,176 (321 tokens stay whole, 35); one head: 512 40 and 44, 16,421 139 and 1,137; fp32, 8 heads:
-// 321 tokens 40 and 47, 2,048 81 and 239.  24 sequences of 1 to 2,500 tokens x 16 heads: 218 and 236.  With the gradients,
-// bf16, 8 heads: 640 tokens 111 and 131, 2,048 162 and 339, 16,421 777 and 2,847 (512 stay whole, 112).
+// Measured, split and whole, in us, calls in a row.  One sequence of 128 x 128: bf16, 8 heads: 512 tokens 42 and 46, 1,024 50
+// and 79, 2,048 69 and 151, 16,421 223 and 1,264 (321 tokens stay whole, 37); one head: 512 41 and 47, 16,421 141 and 1,228;
+// fp32, 8 heads: 321 tokens 39 and 47, 2,048 79 and 237.  The same steps are counted for fewer keys: fp16, 64 x 128, 8 heads:
+// 512 tokens 34 and 45, 4,096 97 and 289; fp32, 64 x 128, 6 heads: 321 tokens 28 and 37.  24 sequences of 1 to 2,500 tokens x
+// 16 heads: 250 and 289 (246 in segments one chunk longer); 8 such: 144 and 224 (131 in longer ones); 64 of 1 to 600 x 8
+// heads stay whole, 129, against 141 in segments of 12.  With the gradients, bf16, 8 heads: 640 tokens 112 and 134, 2,048
+// 163 and 349, 16,421 772 and 2,957 (512 stay whole, 115); 24 packed sequences x 4 heads 315 and 523.
 long long segment_of(OpType t, const DeltaOp& a, bool train) {
     const long long whole = 1LL << 40, C = t == OpType::F32 ? 32 : 64;
     const long long longest = !a.offsets ? a.per_seq : a.max_len > 0 && a.max_len < a.n_tokens ? a.max_len : a.n_tokens;
@@ -1808,7 +1816,7 @@ long long segment_of(OpType t, const DeltaOp& a, bool train) {
     return pick;
 }
 // Eight waves a workgroup share what they read of K, Q and the records, unless four leave no compute unit without work
-// that eight would.  128 segments of 8 chunks x 128 x 128, bf16: 62 us with four, 67 with eight; backward over 192 heads of
+// that eight would.  128 segments of 8 chunks x 128 x 128, bf16: 64 us with four, 67 with eight; backward over 192 heads of
 // 321 tokens x 64 x 128, fp16: 67 with four, 52 with eight.
 bool wide_slices(OpType t, const DeltaOp& a, long long segment) {
     return a.dv > 64 && segments_on_host(a, segment * (t == OpType::F32 ? 32 : 64)) * a.h * 2 > 256;
@@ -1837,9 +1845,12 @@ DeltaSizes delta_sizes(OpType t, const DeltaOp& a, bool train) {
     return s;
 }
 
-// Token by token against chunks at 128 x 128, bf16, in us.  One sequence of 16 heads: 7.2 for one token, 10.1 for 4, 19.6
-// for 12, where a chunk of 13 takes 21.2.  64 such sequences, which fill the chip: 33 for 5 tokens, 63 for 16, 111 for 32,
-// where a chunk of 33 takes 125.
+// Token by token against chunks, in us.  At 128 x 128 in bf16 one sequence of 16 heads: 6.7 for one token, 10.0 for 4, 19.6 for
+// 12, 24 for 16, by chunks 21 for each; 64 such sequences, which fill the chip: 30 for 4 tokens, 61 for 16, 105 for 32, 149 for
+// 48, by chunks 107 to 123.  fp16 and fp32 cross in the same places there (12 tokens 19 and 22, 19.6 and 18; 32 tokens 113 and
+// 128, 110 and 117).  Smaller heads, whose chunks cost less, cross earlier, which the rule does not follow: 64 sequences x 6
+// heads of 64 x 128 in bf16 24 tokens 33 and 34, 32 tokens 42 and 34; x 8 heads of 32 x 32 in fp32 16 tokens 22 and 20, 32
+// tokens 38 and 21.
 bool delta_by_token(const DeltaOp& a) {
     const long long most = (long long)a.n_seqs * a.h >= 256 ? 32 : 12, longest = a.offsets ? a.max_len : a.per_seq;
     return longest <= most && (!a.offsets || a.max_len > 0);

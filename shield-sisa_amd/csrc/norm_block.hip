@@ -10,15 +10,20 @@
 // Both passes are bound by memory: a row is read once into registers, its one or two means are taken there, and every
 // output is written from there.  The backward pass recomputes h from x, z and the residual, which costs what reading h
 // would and needs no saved statistics; it loads the next row before it works on this one.  Where a large copy reaches 5.2
-// TB/s: 246,528 gated rows of 128 in bf16 forward 36 us, 5.3 TB/s; 8,192 rows of 2,048 in bf16 with an fp32 residual 36 us
-// forward (5.6 TB/s) and 62 backward (4.9), 5.5 more for the sums of the weights' gradients.
+// TB/s: 246,528 gated rows of 128 in bf16 forward 36 to 38 us, 5.0 to 5.3 TB/s; 8,192 rows of 2,048 in bf16 with an fp32
+// residual 36 us forward (5.6 TB/s: the caches keep some of it) and 62 backward (4.9), 5.5 more for the sums of the weights'
+// gradients.
 //
 // A row belongs to as many lanes as it has vectors of 8 values (16, 32 or 64 of them, or a workgroup of its own): few
 // registers, many rows in flight.  With several vectors a lane and at most a wave a row, the gated rows of 128 took 44 us
 // and a training step on the rows of 2,048 154, against 36 and 107.  The vectors need no more than their element's alignment
 // (gfx950 takes any), so odd strides cost a split line, not another path: 10,272 rows of 385 in fp16 take 12 us forward (3.3
-// TB/s) and 24 backward.  Where 8 does not divide the row, its last lane's vector ends at the row's end and repeats values
-// of the lane before: both compute and write them alike, and only the sums leave the second copy out.
+// TB/s) and 24 backward.  Narrower rows than 128 leave some of their 16 lanes without values, and the vector units, 81 % busy
+// at 128, then bound: 31.6 million gated values in bf16 take 32 us in rows of 128, 49 in rows of 64, 90 of 32 and 178 of 16.
+// Backward, rows of more than 4,096 take 1,024 threads of 128 registers, 10 to 12 of which spill with rows of two bytes and 57
+// to 70 with fp32 ones: 15.8 million values with all parts in bf16 with an fp32 residual 95 us in rows of 4,096 (forward and
+// backward), 207 in rows of 8,192.  Where 8 does not divide the row, its last lane's vector ends at the row's end and repeats
+// values of the lane before: both compute and write them alike, and only the sums leave the second copy out.
 #include "dev_common.hpp"
 #include "ops.hpp"
 

@@ -765,6 +765,7 @@ template <typename T, int NK, int W, bool TRAIN, bool WHOLE>
 __global__ void __launch_bounds__(64 * W) delta_transit_kernel(DeltaOp a) {
     typedef Record<T> R;
     typedef Feed<T, NK, W, WHOLE, false, R::A_AT> Reader;   // T and the vectors: A is not needed
+    static_assert(Reader::TWO_X, "one stage of X needs xs_read");
     constexpr int C = R::C, NT = R::NT, NP = R::NP, P = Parts<T>::IN, M = 2 * NK;
     constexpr int COLUMNS = M * NK * MID * kBlock;
     __shared__ __attribute__((aligned(1024))) unsigned char mem[Reader::BYTES > COLUMNS ? Reader::BYTES : COLUMNS];
@@ -1263,6 +1264,7 @@ __global__ void __launch_bounds__(64 * W) delta_back_kernel(DeltaOp a, DeltaGrad
     typedef Record<T> R;
     constexpr int C = R::C, NT = R::NT, NP = R::NP, P = Parts<T>::IN, M = 2 * NK;
     typedef Feed<T, NK, W, WHOLE, true, R::BYTES> Reader;
+    static_assert(Reader::TWO_X, "one stage of X needs xs_read");
     __shared__ __attribute__((aligned(1024))) unsigned char mem[Reader::BYTES];
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
